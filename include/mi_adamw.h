@@ -467,8 +467,9 @@ int mi_adamw_probe_flat(const mi_adamw_tensor *t, int64_t chunk_elems, int32_t s
 
 /* How the products of a Newton-Schulz step are formed, all on the fp16 matrix cores with
  * fp32 sums.  HALF: fp16 operands, the iterate carried in two fp16 terms and the diagonals of
- * the square factors in fp32: 2e-4 to 8e-4 relative to 64 bits, below the rounding of a bf16
- * result.  SINGLE: every operand in two terms, three products: fp32's error. */
+ * the square factors in fp32: 3e-4 to 7e-4 relative to 64 bits on gradients' spectra, below the
+ * rounding of a bf16 result; up to 2e-3 for low ranks, 4e-3 where a handful of entries is not
+ * zero.  SINGLE: every operand in two terms, three products: fp32's error. */
 #define MI_ADAMW_NS_HALF 0
 #define MI_ADAMW_NS_SINGLE 1
 

@@ -15,10 +15,14 @@
 //           counts.  X is carried in two fp16 terms (22 bits), since a^5 = 485 multiplies the
 //           rounding of small singular directions; the product reads the first term.  The
 //           diagonals of S and P, their largest entries, are held apart in fp32 and enter the
-//           elementwise part.  Against 64 bits, relative: 2e-4 to 8e-4 on gradients' spectra,
-//           below the 1.7e-3 of rounding the result to bf16 (1e-3 to 6e-3 without the two).
-//   single  every operand in two fp16 terms, hi hi + hi lo + lo hi: fp32's error (2e-6 to
-//           1e-5 against 64 bits, as the same iteration in fp32 has).
+//           elementwise part.  Against 64 bits, relative: 3e-4 to 7e-4 on gradients' spectra
+//           and full ranks, below the 1.7e-3 of rounding the result to bf16 (1e-3 to 6e-3
+//           without the two); up to 2e-3 for low ranks, dense or in few rows, and 4e-3 where a
+//           handful of entries is all there is, since nothing averages their roundings.
+//           (The same iteration in bf16: 1e-2 to 2e-2, and 0.1 to 1.6 for low ranks.)
+//   single  every operand in two fp16 terms, hi hi + hi lo + lo hi: fp32's error (1e-6 against
+//           64 bits on gradients' spectra, up to 1.4e-4 at rank one, as the same iteration in
+//           fp32 has).
 //
 // X is stored as its transpose T [n][m] alone, padded with zeros to multiples of 64, which every
 // product keeps zero.  P X reads it with its summed index contiguous; X X^T sums over T's rows and
@@ -61,7 +65,8 @@ struct Quintic {
 // Where the parts of one matrix's workspace lie, in bytes from its beginning.
 struct Layout {
     int32_t m, n, mp, np;
-    int64_t t, s, p, ds, dp, parts, counts, bytes;
+    int64_t t, s, p, ds, dp, counts, bytes;
+    int64_t parts;                  // shares of the norm, then of P's trace
     int64_t t_lo, sq_lo;            // from a first term to its second
     int64_t t_turn;                 // from the transpose one step reads to the next one's
 };
@@ -508,7 +513,7 @@ __host__ __device__ __forceinline__ void triangle_tile(int32_t k, int32_t down, 
 
 template <class Src, int kPhase, bool kSingle, int kT, int kLanes = Shape<kT, kSingle>::kWaves * 64>
 __global__ __launch_bounds__(kLanes) void mi_adamw_ns_product_kernel(
-    Src src, Quintic f, char* ws, int32_t turn, int32_t want_split, MuonOut o) {
+    Src src, Quintic f, char* ws, int32_t turn, int32_t want, MuonOut o) {
     typedef Shape<kT, kSingle> W;
     constexpr bool kPair = kPhase == kPhaseS || kPhase == kPhaseP;
     constexpr bool kSum = kPhase == kPhaseS;
@@ -520,7 +525,7 @@ __global__ __launch_bounds__(kLanes) void mi_adamw_ns_product_kernel(
     char* base = ws + it.mat.workspace;
     const int32_t down = (l.mp + kT - 1) / kT;
     int32_t ti, tj;
-    const int32_t split = kPair ? split_of(l, kT, want_split) : 1;
+    const int32_t split = kPair ? split_of(l, kT, want) : 1;
     const int32_t part = kPair ? it.index % split : 0;
     if (kPhase == kPhaseP && part) return;      // P's sums are short
     if (kPair) triangle_tile(it.index / split, down, ti, tj);
@@ -642,6 +647,11 @@ __global__ __launch_bounds__(kLanes) void mi_adamw_ns_product_kernel(
             for (int q = 0; q < kFj; ++q) f.b[term][q] = read_one(step, kk, 1, term, q);
         }
     };
+    // P's trace over m in half precision, from the shares that P's tiles on the diagonal left
+    // (`want`: their side): asked for here, used after the product.
+    const float* traces = reinterpret_cast<const float*>(base + l.parts);
+    const int32_t n_traces = kPair || kSingle ? 0 : (l.mp + want - 1) / want;
+    float trace = lane < n_traces ? *(const GLOBAL float*)(traces + lane) : 0.0f;
     f32x4 acc[kFi][kFj] = {};
     auto multiply = [&](const Fragments& f) {
 #pragma unroll
@@ -801,6 +811,7 @@ __global__ __launch_bounds__(kLanes) void mi_adamw_ns_product_kernel(
                 for (int e = 0; e < 4; ++e)
                     if (i + e == j) {
                         diag[j] = v[e];
+                        trace += v[e];
                         v[e] = 0.0f;
                     }
                 for (int e = 0; e < 4; ++e) v[e] *= kPhase == kPhaseS ? kScaleS : kScaleP;
@@ -810,7 +821,21 @@ __global__ __launch_bounds__(kLanes) void mi_adamw_ns_product_kernel(
                 *(GLOBAL half4*)(to + mirrored) = hi;
                 if (kSingle) *(GLOBAL half4*)(to + l.sq_lo + mirrored) = lo;
             }
-        if (ti == tj) return;
+        if (ti == tj) {
+            if (kPhase == kPhaseP && !kSingle) {
+                // the tile's share of P's trace
+                for (int d = 32; d > 0; d >>= 1) trace += __shfl_xor(trace, d);
+                float* sums = reinterpret_cast<float*>(lds);
+                __syncthreads();
+                if (lane == 0) sums[wave] = trace;
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    for (int w = 1; w < W::kWaves; ++w) trace += sums[w];
+                    reinterpret_cast<float*>(base + l.parts)[ti] = trace;
+                }
+            }
+            return;
+        }
         // the other triangle: the tile turned round in LDS
 #pragma unroll
         for (int term = 0; term < kTerms; ++term) {
@@ -836,8 +861,19 @@ __global__ __launch_bounds__(kLanes) void mi_adamw_ns_product_kernel(
         }
         return;
     }
-    // X' = (a + D) X + P' X, P' = off the diagonal.  Four of a wave's lanes write a line of 32 kG
-    // bytes; as the sides are padded to multiples of 64, a lane's values are all there or none.
+    // X' = (a + D) X + P' X, P' = off the diagonal.  In half precision P' reads X's first term, so D
+    // takes the second one at its mean alone: what D_i - D_k of the rounding would add beyond P's own
+    // product points out of the rows that X has, where the steps to come amplify it (of rank one in 2
+    // of 256 rows the result was 4e-2 off with D_i there, and is 2e-3; with no D at all a full rank's
+    // 7e-4 would be 1.3e-3).
+    // Four of a wave's lanes write a line of 32 kG bytes; as the sides are padded to multiples of 64,
+    // a lane's values are all there or none.
+    float second = 0.0f;
+    if (!kSingle) {
+        for (int32_t k = lane + 64; k < n_traces; k += 64) trace += traces[k];
+        for (int d = 32; d > 0; d >>= 1) trace += __shfl_xor(trace, d);
+        second = f.a + trace / l.m;
+    }
 #pragma unroll
     for (int fb = 0; fb < kFi / kG; ++fb) {
         const int32_t i = row_of(fb * kG);
@@ -858,10 +894,13 @@ __global__ __launch_bounds__(kLanes) void mi_adamw_ns_product_kernel(
                 half8 hi, lo;
                 for (int e = 0; e < 8; ++e) {
                     const int fi = fb * kG + q * 2 + e / 4;
-                    const float x = static_cast<float>(old[fb][fj][q][0][e]) +
-                                    static_cast<float>(old[fb][fj][q][1][e]);
-                    const float v = __builtin_fmaf(d[q * 2 + e / 4][e % 4], x,
-                                                   acc[fi][fj][e % 4] * (1.0f / kScaleP));
+                    const float x0 = static_cast<float>(old[fb][fj][q][0][e]);
+                    const float x1 = static_cast<float>(old[fb][fj][q][1][e]);
+                    const float di = d[q * 2 + e / 4][e % 4];
+                    const float px = acc[fi][fj][e % 4] * (1.0f / kScaleP);
+                    const float v =
+                        kSingle ? __builtin_fmaf(di, x0 + x1, px)
+                                : __builtin_fmaf(di, x0, __builtin_fmaf(second, x1, px));
                     hi[e] = static_cast<_Float16>(v);
                     lo[e] = static_cast<_Float16>(v - static_cast<float>(hi[e]));
                     if (kPhase == kPhaseLast) acc[fi][fj][e % 4] = v * (1.0f / kScaleX);
@@ -1256,24 +1295,26 @@ struct Cut {
 };
 
 template <class Src, int kPhase, bool kSingle, int kT>
-void launch_tiles(const Src& src, unsigned grid, Quintic f, char* ws, int32_t turn, int32_t split,
+void launch_tiles(const Src& src, unsigned grid, Quintic f, char* ws, int32_t turn, int32_t want,
                   const MuonOut& o, hipStream_t s) {
     hipLaunchKernelGGL((mi_adamw_ns_product_kernel<Src, kPhase, kSingle, kT>), dim3(grid),
-                       dim3(Shape<kT, kSingle>::kWaves * 64), 0, s, src, f, ws, turn, split, o);
+                       dim3(Shape<kT, kSingle>::kWaves * 64), 0, s, src, f, ws, turn, want, o);
 }
 
 template <class Src, int kPhase, bool kSingle>
 void launch_product(const Src& src, unsigned grid, const Cut& cut, Quintic f, char* ws,
                     int32_t turn, const MuonOut& o, hipStream_t s) {
-    const int32_t tile = kPhase == kPhaseS || kPhase == kPhaseP ? cut.pair_tile : cut.tile;
+    constexpr bool kPair = kPhase == kPhaseS || kPhase == kPhaseP;
+    const int32_t tile = kPair ? cut.pair_tile : cut.tile;
+    const int32_t want = kPair ? cut.split : cut.pair_tile;
     if (tile == 256)
-        return launch_tiles<Src, kPhase, kSingle, 256>(src, grid, f, ws, turn, cut.split, o, s);
+        return launch_tiles<Src, kPhase, kSingle, 256>(src, grid, f, ws, turn, want, o, s);
     if constexpr (!kSingle) {
         if (tile == 192)
-            return launch_tiles<Src, kPhase, kSingle, 192>(src, grid, f, ws, turn, cut.split, o, s);
+            return launch_tiles<Src, kPhase, kSingle, 192>(src, grid, f, ws, turn, want, o, s);
     }
-    if (tile == 128) launch_tiles<Src, kPhase, kSingle, 128>(src, grid, f, ws, turn, cut.split, o, s);
-    else launch_tiles<Src, kPhase, kSingle, 64>(src, grid, f, ws, turn, cut.split, o, s);
+    if (tile == 128) launch_tiles<Src, kPhase, kSingle, 128>(src, grid, f, ws, turn, want, o, s);
+    else launch_tiles<Src, kPhase, kSingle, 64>(src, grid, f, ws, turn, want, o, s);
 }
 
 // source_of(kind): the launch's source, and its grid.
