@@ -153,14 +153,17 @@ class _Batch:
     """The device tables of matrices that are stepped by one sequence of launches."""
 
     __slots__ = ("params", "rows", "host_rows", "matrices", "items", "tables", "options",
-                 "workspace", "recorded")
+                 "workspace", "recorded", "kept", "__weakref__")
 
     def __init__(self, entries, options: _lib.NsOptions, adjust, copies, device):
         """entries: (parameter, gradient, momentum) triples."""
         lib = _lib.load()
         self.params = [p for p, _, _ in entries]
         self.options = options
-        self.recorded = False       # a graph reads these tables, which then never change
+        # What graphs read, once a step was recorded: their end is not announced, so it stays.
+        # `recorded`: the present rows are among it, and then never change.
+        self.kept: list = []
+        self.recorded = False
         n = len(entries)
         rows = np.zeros(n, dtype=_ROW_DTYPE)
         rows["param"] = [p.data_ptr() for p in self.params]
@@ -198,17 +201,24 @@ class _Batch:
             self.tables.items[kind] = self.items[-1].data_ptr()
             self.tables.n_items[kind] = count
 
-    def move_grads(self, grads: np.ndarray, device: torch.device, stream: int):
+    def record(self, entries) -> None:
+        """A graph's launches take these tables, and with them the tensors whose addresses
+        they hold: parameter, gradient, momentum and copy of each entry."""
+        if not self.recorded:
+            self.recorded = True
+            self.kept.append((self.rows, entries))
+
+    def move_grads(self, grads: np.ndarray, device: torch.device, stream: int) -> None:
         """The gradients lie elsewhere: their addresses go to the device as kernel arguments,
-        or in new rows where a graph reads the old ones, which are returned to be kept."""
+        or in new rows where a graph reads the old ones."""
         idx = np.flatnonzero(grads != self.host_rows["grad"]).astype(np.int32)
         if not len(idx):
-            return None
+            return
         if self.recorded:
-            old, self.recorded = self.rows, False
+            self.recorded = False
             self.host_rows["grad"] = grads
             self.rows = _upload(self.host_rows, device)
-            return old
+            return
         moved = np.ascontiguousarray(grads[idx])
         vec = np.zeros(len(idx), dtype=np.uint8)
         code = _lib.load().mi_adamw_set_grads(self.rows.data_ptr(), len(self.host_rows), len(idx),
@@ -216,7 +226,6 @@ class _Batch:
                                               vec.ctypes.data, stream)
         self.host_rows["grad"] = grads if code == _lib.OK else 0
         _lib.check(code, "mi_adamw_set_grads")
-        return None
 
 
 def _original(rows: int, cols: int) -> float:
@@ -490,8 +499,7 @@ class Muon(Optimizer):
         if key != self._key:
             self._key = None
             new = self._build(groups, device)
-            # what a graph reads stays: its end is not announced
-            self._kept += [b for batches in self._batches for b in batches if b.recorded]
+            self._kept += [b for batches in self._batches for b in batches if b.kept]
             self._batches = new
             self._key = key
         lib = _lib.load()
@@ -508,11 +516,10 @@ class Muon(Optimizer):
                 if capturing:
                     if not np.array_equal(grads, b.host_rows["grad"]):
                         self._refuse_capture()
-                    b.recorded = True
+                    b.record([(p.detach(), p.grad, self.state[p]["momentum_buffer"],
+                               self._copies.get(id(p))) for p in b.params])
                 else:
-                    old = b.move_grads(grads, device, stream)
-                    if old is not None:
-                        self._kept.append(old)
+                    b.move_grads(grads, device, stream)
                 _lib.check(lib.mi_adamw_muon_step(
                     b.rows.data_ptr(), b.matrices.data_ptr(), ctypes.addressof(b.tables),
                     ctypes.addressof(hyper), ctypes.addressof(b.options), flags, ws.data_ptr(),

@@ -1,0 +1,83 @@
+"""Muon steps recorded into HIP graphs, replayed between eager steps that move gradients and rebuild
+tables: every replay equals an eager step of a twin with the recorded gradients, bit for bit."""
+import copy
+
+import pytest
+import torch
+
+import mi_adamw
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+SHAPES = [(96, 64), (300, 180), (200, 200), (64, 520)]
+
+
+def make(seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return [torch.nn.Parameter(0.02 * torch.randn(s, device=DEV, generator=g)) for s in SHAPES]
+
+
+def set_grads(params, seed):
+    g = torch.Generator(device=DEV).manual_seed(100 + seed)
+    for p in params:
+        p.grad = 1e-3 * torch.randn(p.shape, device=DEV, generator=g)
+
+
+def twin_of(opt, params, **options):
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    twin = mi_adamw.Muon(twins, **options)
+    twin.load_state_dict(copy.deepcopy(opt.state_dict()))
+    return twin, twins
+
+
+def eager(opt, params, grads):
+    for p, g in zip(params, grads):
+        p.grad = None if g is None else g.clone()
+    opt.step()
+
+
+def occupy():
+    """Memory that was freed is taken and written over."""
+    junk = [torch.full((n,), 0x7b, dtype=torch.uint8, device=DEV)
+            for n in (512, 512, 2048, 4096, 1 << 16) * 20]
+    torch.cuda.synchronize()
+    return junk
+
+
+def same(params, twins):
+    return all(torch.equal(p, q) for p, q in zip(params, twins))
+
+
+def test_replays_after_moved_gradients_and_rebuilt_tables():
+    options = dict(lr=0.02)
+    params = make()
+    opt = mi_adamw.Muon(params, **options)
+    set_grads(params, 0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            opt.step()
+        recorded = [p.grad.clone() for p in params]
+        twin, twins = twin_of(opt, params, **options)
+        for k in range(3):
+            set_grads(params, 2 * k + 1)                # moved
+            grads = [p.grad for p in params]
+            opt.step()
+            eager(twin, twins, grads)
+            set_grads(params, 2 * k + 2)
+            params[k].grad = None                       # other tables
+            grads = [p.grad for p in params]
+            opt.step()
+            eager(twin, twins, grads)
+            assert same(params, twins)
+            junk = occupy()
+            graph.replay()
+            eager(twin, twins, recorded)
+            torch.cuda.synchronize()
+            assert same(params, twins)
+            del junk
+    torch.cuda.current_stream().wait_stream(side)
