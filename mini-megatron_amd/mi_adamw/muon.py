@@ -153,13 +153,14 @@ class _Batch:
     """The device tables of matrices that are stepped by one sequence of launches."""
 
     __slots__ = ("params", "rows", "host_rows", "matrices", "items", "tables", "options",
-                 "workspace", "recorded", "kept", "__weakref__")
+                 "workspace", "stream", "rows_stream", "recorded", "kept", "__weakref__")
 
-    def __init__(self, entries, options: _lib.NsOptions, adjust, copies, device):
-        """entries: (parameter, gradient, momentum) triples."""
+    def __init__(self, entries, options: _lib.NsOptions, adjust, copies, device, stream: int):
+        """entries: (parameter, gradient, momentum) triples; stream: the current one."""
         lib = _lib.load()
         self.params = [p for p, _, _ in entries]
         self.options = options
+        self.stream = self.rows_stream = stream     # where the tables and the rows were allocated
         # What graphs read, once a step was recorded: their end is not announced, so it stays.
         # `recorded`: the present rows are among it, and then never change.
         self.kept: list = []
@@ -201,12 +202,29 @@ class _Batch:
             self.tables.items[kind] = self.items[-1].data_ptr()
             self.tables.n_items[kind] = count
 
+    def used_on(self, stream: int, device: torch.device) -> None:
+        """An eager launch on `stream` reads the tables.  A program orders the steps of the same
+        parameters on different streams, and so the tables' contents; their memory has to outlast
+        what is queued on streams other than the one it was allocated on."""
+        if device.type != "cuda" or stream == self.stream == self.rows_stream:
+            return
+        current = torch.cuda.current_stream(device)
+        for t, home in ((self.rows, self.rows_stream), (self.matrices, self.stream),
+                        *((t, self.stream) for t in self.items)):
+            if t is not None and home != stream:
+                t.record_stream(current)
+
     def record(self, entries) -> None:
         """A graph's launches take these tables, and with them the tensors whose addresses
         they hold: parameter, gradient, momentum and copy of each entry."""
         if not self.recorded:
             self.recorded = True
             self.kept.append((self.rows, entries))
+
+    def grads(self) -> np.ndarray:
+        """The addresses of the gradients now."""
+        return np.fromiter((p.grad.data_ptr() for p in self.params), dtype=np.uint64,
+                           count=len(self.params))
 
     def move_grads(self, grads: np.ndarray, device: torch.device, stream: int) -> None:
         """The gradients lie elsewhere: their addresses go to the device as kernel arguments,
@@ -217,7 +235,7 @@ class _Batch:
         if self.recorded:
             self.recorded = False
             self.host_rows["grad"] = grads
-            self.rows = _upload(self.host_rows, device)
+            self.rows, self.rows_stream = _upload(self.host_rows, device), stream
             return
         moved = np.ascontiguousarray(grads[idx])
         vec = np.zeros(len(idx), dtype=np.uint8)
@@ -256,8 +274,8 @@ class Muon(Optimizer):
                   ``mi_adamw.bf16_weights``.
 
     Parameters are 2-D, contiguous, fp32 and on one ROCm GPU, as are their gradients.  A step
-    may be recorded into a HIP graph once an eager one has built its tables with the
-    gradients in place; the learning rate is recorded as its value.
+    may be recorded into a HIP graph, on any stream, once an eager one has built its tables
+    with the gradients in place; the learning rate is recorded as its value.
     """
 
     def __init__(self, params, lr: float | torch.Tensor = 1e-3, weight_decay: float = 0.1,
@@ -422,10 +440,8 @@ class Muon(Optimizer):
                            "the last eager step; run one eager step with the same parameters, "
                            "gradient tensors, state and options before capturing")
 
-    def _build(self, groups, device) -> list[list[_Batch]]:
+    def _build(self, groups, device, stream: int) -> list[list[_Batch]]:
         """Each group's matrices, by precision, in batches whose workspace stays bounded."""
-        if torch.cuda.is_current_stream_capturing():
-            self._refuse_capture()
         lib = _lib.load()
         built = []
         for group, entries in zip(self.param_groups, groups):
@@ -451,11 +467,12 @@ class Muon(Optimizer):
                                                   f"{tuple(e[0].shape)} is too large")
                     if batch and size + need > _WORKSPACE:
                         built[-1].append(_Batch(batch, options, adjust, self._copies_or_none(),
-                                                device))
+                                                device, stream))
                         batch, size = [], 0
                     batch.append(e)
                     size += need
-                built[-1].append(_Batch(batch, options, adjust, self._copies_or_none(), device))
+                built[-1].append(_Batch(batch, options, adjust, self._copies_or_none(), device,
+                                        stream))
         return built
 
     def _copies_or_none(self):
@@ -483,6 +500,7 @@ class Muon(Optimizer):
         return loss
 
     def _launch(self, groups, device) -> None:
+        capturing = torch.cuda.is_current_stream_capturing()
         if self.bf16_copy:
             for entries in groups:
                 for p, _, _ in entries:
@@ -490,15 +508,18 @@ class Muon(Optimizer):
                     if c is None or c.shape != p.shape or c.device != device:
                         self._refresh_copy(p)
         stream = torch._C._cuda_getCurrentRawStream(device.index)
-        key = (stream, self.ns_precision,
+        key = (self.ns_precision,
                [(g["adjust_lr_fn"], tuple(g["ns_coefficients"]), g["eps"], g["ns_steps"])
                 for g in self.param_groups],
                [[(p.data_ptr(), m.data_ptr(), p.shape) for p, _, m in entries]
                 for entries in groups])
-        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and (key != self._key or any(
+                not np.array_equal(b.grads(), b.host_rows["grad"])
+                for batches in self._batches for b in batches)):
+            self._refuse_capture()
         if key != self._key:
             self._key = None
-            new = self._build(groups, device)
+            new = self._build(groups, device, stream)
             self._kept += [b for batches in self._batches for b in batches if b.kept]
             self._batches = new
             self._key = key
@@ -511,15 +532,12 @@ class Muon(Optimizer):
             hyper = _lib.MuonHyper(1 - momentum, momentum, bool(group["nesterov"]),
                                    1 - lr * group["weight_decay"], -lr)
             for b in batches:
-                grads = np.fromiter((p.grad.data_ptr() for p in b.params), dtype=np.uint64,
-                                    count=len(b.params))
                 if capturing:
-                    if not np.array_equal(grads, b.host_rows["grad"]):
-                        self._refuse_capture()
                     b.record([(p.detach(), p.grad, self.state[p]["momentum_buffer"],
                                self._copies.get(id(p))) for p in b.params])
                 else:
-                    b.move_grads(grads, device, stream)
+                    b.move_grads(b.grads(), device, stream)
+                    b.used_on(stream, device)
                 _lib.check(lib.mi_adamw_muon_step(
                     b.rows.data_ptr(), b.matrices.data_ptr(), ctypes.addressof(b.tables),
                     ctypes.addressof(hyper), ctypes.addressof(b.options), flags, ws.data_ptr(),

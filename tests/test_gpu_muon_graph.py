@@ -81,3 +81,49 @@ def test_replays_after_moved_gradients_and_rebuilt_tables():
             assert same(params, twins)
             del junk
     torch.cuda.current_stream().wait_stream(side)
+
+
+def test_plain_capture_after_eager_steps_on_the_default_stream():
+    """The usual order: eager steps on the current stream, then torch.cuda.graph(), which captures
+    on a stream of its own."""
+    options = dict(lr=0.02, bf16_copy=True)
+    params = make(1)
+    opt = mi_adamw.Muon(params, **options)
+    set_grads(params, 0)
+    opt.step()
+    twin, twins = twin_of(opt, params, **options)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for k in range(4):
+        for p in params:
+            p.grad.mul_(-0.5)
+        graph.replay()
+        eager(twin, twins, [p.grad for p in params])
+        torch.cuda.synchronize()
+        assert same(params, twins)
+        assert all(torch.equal(opt.bf16_param(p), p.detach().bfloat16()) for p in params)
+
+
+def test_streams_in_turn():
+    options = dict(lr=0.02)
+    params = make(2)
+    opt = mi_adamw.Muon(params, **options)
+    twin, twins = twin_of(opt, params, **options)
+    streams = [torch.cuda.current_stream(), torch.cuda.Stream(), torch.cuda.Stream()]
+    for k in range(7):
+        stream, last = streams[k % 3], streams[(k - 1) % 3]
+        stream.wait_stream(last)
+        with torch.cuda.stream(stream):
+            set_grads(params, k)
+            if k == 4:
+                params[1].grad = None                   # other tables, the old ones still queued
+            opt.step()
+            junk = occupy() if k == 5 else None
+    torch.cuda.synchronize()
+    for k in range(7):
+        set_grads(twins, k)
+        if k == 4:
+            twins[1].grad = None
+        twin.step()
+    assert same(params, twins)

@@ -158,3 +158,50 @@ def test_tables_that_no_graph_reads_end(machine):
     step(opt)
     gc.collect()
     assert all(t() is None for t in tables) and not opt._kept
+
+
+def batches(opt):
+    return [b for of_group in opt._batches for b in of_group]
+
+
+def test_a_capture_on_another_stream(machine):
+    """torch.cuda.graph() captures on a stream of its own."""
+    opt, params = optimizer(bf16_copy=True)
+    step(opt)
+    built = batches(opt)
+    machine.stream = 7
+    read = capture(opt, machine)
+    assert batches(opt) == built and {s["stream"] for s in machine.lib.steps} == {0, 7}
+    machine.stream = 0
+    move(params)
+    step(opt)
+    assert batches(opt) == built and alive(read)
+
+
+def test_streams_in_turn_build_nothing(machine):
+    opt, params = optimizer()
+    step(opt)
+    built = batches(opt)
+    for machine.stream in (1, 0, 2, 1):
+        step(opt)
+        move(params)
+    assert batches(opt) == built
+
+
+def test_a_refused_capture_leaves_the_tables(machine):
+    opt, params = optimizer()
+    step(opt)
+    built = batches(opt)
+    kept = [p.grad for p in params]
+    params[0].grad = torch.randn(params[0].shape)
+    before = len(machine.lib.steps)
+    with pytest.raises(RuntimeError, match="under graph capture"):
+        capture(opt, machine)
+    opt.param_groups[0]["ns_steps"] = 3
+    with pytest.raises(RuntimeError, match="under graph capture"):
+        capture(opt, machine)
+    opt.param_groups[0]["ns_steps"] = 5
+    assert len(machine.lib.steps) == before and not any(b.kept for b in built)
+    params[0].grad = kept[0]
+    step(opt)
+    assert batches(opt) == built
