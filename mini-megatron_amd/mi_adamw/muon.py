@@ -506,6 +506,8 @@ class Muon(Optimizer):
                 for p, _, _ in entries:
                     c = self._copies.get(id(p))
                     if c is None or c.shape != p.shape or c.device != device:
+                        if capturing:
+                            self._refuse_capture()
                         self._refresh_copy(p)
         stream = torch._C._cuda_getCurrentRawStream(device.index)
         key = (self.ns_precision,

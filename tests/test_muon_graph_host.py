@@ -205,3 +205,12 @@ def test_a_refused_capture_leaves_the_tables(machine):
     params[0].grad = kept[0]
     step(opt)
     assert batches(opt) == built
+
+
+def test_a_capture_without_its_copies_is_refused(machine):
+    opt, params = optimizer(bf16_copy=True)
+    step(opt)
+    opt._copies.clear()
+    with pytest.raises(RuntimeError, match="under graph capture"):
+        capture(opt, machine)
+    assert not opt._copies
