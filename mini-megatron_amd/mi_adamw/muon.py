@@ -108,7 +108,8 @@ def newton_schulz(x: torch.Tensor, *, steps: int = 5, coefficients=NS_COEFFICIEN
     if out is not None and (out.shape != x.shape or out.dtype != x.dtype
                             or out.device != x.device):
         raise ValueError("newton_schulz: out needs x's shape, dtype and device")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(x)
     if x.numel() == 0:
         return out
@@ -146,6 +147,8 @@ def newton_schulz(x: torch.Tensor, *, steps: int = 5, coefficients=NS_COEFFICIEN
             "mi_adamw_newton_schulz")
     if to is not o3:
         o3.copy_(to)
+    elif given:
+        torch.autograd.graph.increment_version(out)     # as an operator that writes it in place
     return out
 
 

@@ -1,0 +1,47 @@
+"""newton_schulz's out=: autograd sees the write, memory that out shares with x, and large batches."""
+import pytest
+import torch
+
+import mi_adamw
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+SINGLE = 199 * 3 * 2.0 ** -23            # derived in test_gpu_newton_schulz.py
+
+
+def normal(*shape, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.randn(*shape, device=DEV, generator=g)
+
+
+@pytest.mark.parametrize("shape", [(20, 30), (200, 300), (3, 20, 30)])
+@pytest.mark.parametrize("layout", ["itself", "dense", "columns dense", "strided"])
+def test_out_is_seen_by_autograd(shape, layout):
+    x = normal(*shape)
+    if layout == "itself":
+        out = x
+    elif layout == "dense":
+        out = torch.empty_like(x)
+    elif layout == "columns dense":
+        out = torch.empty_like(x.mT.contiguous()).mT
+    else:
+        out = torch.empty(*shape, 2, device=DEV)[..., 0]
+    w = torch.ones_like(x, requires_grad=True)
+    product = (w * out).sum()               # saves out for w's gradient
+    version = out._version
+    mi_adamw.newton_schulz(x, out=out)
+    assert out._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+
+
+def test_x_alone_is_not_written():
+    x = normal(40, 50)
+    version = x._version
+    mi_adamw.newton_schulz(x)
+    assert x._version == version
+    with torch.inference_mode():            # tensors without a version
+        y = torch.empty_like(x)
+        mi_adamw.newton_schulz(x, out=y)
+    assert torch.equal(y, mi_adamw.newton_schulz(x))
