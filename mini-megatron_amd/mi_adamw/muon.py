@@ -549,6 +549,7 @@ class Muon(Optimizer):
                     stream), "mi_adamw_muon_step")
         for entries in groups:
             for p, _, m in entries:
-                torch.autograd.graph.increment_version(p)
+                copy = (self._copies[id(p)],) if self.bf16_copy else ()
+                torch.autograd.graph.increment_version((p, m, *copy))
                 if self._copy_sync is not None:
                     self._copy_sync[id(p)] = (p._version, p.data_ptr())

@@ -127,3 +127,24 @@ def test_streams_in_turn():
             twins[1].grad = None
         twin.step()
     assert same(params, twins)
+
+
+def test_a_backward_through_stepped_copies_raises():
+    """The forward of bf16_weights saves the copies that the step writes."""
+    model = torch.nn.Sequential(torch.nn.Linear(64, 96, bias=False),
+                                torch.nn.Linear(96, 64, bias=False)).to(DEV)
+    opt = mi_adamw.Muon(model.parameters(), lr=0.02, bf16_copy=True)
+    x = torch.randn(8, 64, device=DEV)
+
+    def forward():
+        with torch.autocast("cuda", dtype=torch.bfloat16), mi_adamw.bf16_weights(opt, model):
+            return model(x).float().square().mean()
+
+    forward().backward()
+    late = forward()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified (by an )?inplace"):
+        late.backward()
+    opt.zero_grad()
+    forward().backward()
+    opt.step()

@@ -214,3 +214,17 @@ def test_a_capture_without_its_copies_is_refused(machine):
     with pytest.raises(RuntimeError, match="under graph capture"):
         capture(opt, machine)
     assert not opt._copies
+
+
+def test_a_step_raises_the_versions_of_all_it_writes(machine):
+    opt, params = optimizer(bf16_copy=True)
+    written = [t for p in params
+               for t in (p, opt.state[p]["momentum_buffer"], opt.bf16_param(p))]
+    for _ in range(2):
+        before = [t._version for t in written]
+        step(opt)
+        assert all(t._version > v for t, v in zip(written, before))
+    params[0].grad = None
+    before = params[0]._version
+    step(opt)
+    assert params[0]._version == before
