@@ -85,6 +85,16 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(1) if t.shape[1] > 1 else t.shape[2]
 
 
+def _overlap(x: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether writing a matrix of a 3-D out may change another one of x before it is read: out
+    shares memory with x and is not the same view.  (Each matrix is read before it is written.)"""
+    if x.shape[0] == 1 or (x.data_ptr() == out.data_ptr() and x.stride() == out.stride()):
+        return False
+    ends = [t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in
+                                                       zip(t.shape, t.stride()))) for t in (x, out)]
+    return x.data_ptr() < ends[1] and out.data_ptr() < ends[0]
+
+
 @torch.no_grad()
 def newton_schulz(x: torch.Tensor, *, steps: int = 5, coefficients=NS_COEFFICIENTS,
                   eps: float = 1e-7, precision: str | None = None,
@@ -94,7 +104,8 @@ def newton_schulz(x: torch.Tensor, *, steps: int = 5, coefficients=NS_COEFFICIEN
     x:          fp32 or bf16 on a ROCm GPU, 2-D or 3-D; rows or columns dense at any stride
                 (other layouts are copied first).  It is not differentiable.
     precision:  "half", "single", or None: single for fp32, half for bf16.
-    out:        where the result goes (same shape, dtype and device; may be x itself).
+    out:        where the result goes (same shape, dtype and device; may be x itself or share
+                memory with it).
     """
     if x.dim() not in (2, 3):
         raise ValueError(f"newton_schulz takes a matrix or a batch of them, got {x.dim()} "
@@ -121,8 +132,9 @@ def newton_schulz(x: torch.Tensor, *, steps: int = 5, coefficients=NS_COEFFICIEN
         else:
             x3 = x3 if _rows_dense(x3) else x3.contiguous()
     to = o3
-    if not _rows_dense(o3) or (o3.shape[0] > 1 and
-                               o3.stride(0) < (o3.shape[1] - 1) * _row_stride(o3) + o3.shape[2]):
+    if not _rows_dense(o3) or _overlap(x3, o3) or (
+            o3.shape[0] > 1 and
+            o3.stride(0) < (o3.shape[1] - 1) * _row_stride(o3) + o3.shape[2]):
         to = torch.empty(o3.shape, dtype=o3.dtype, device=o3.device)
     batch, rows, cols = x3.shape
     lib = _lib.load()

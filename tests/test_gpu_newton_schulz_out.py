@@ -45,3 +45,19 @@ def test_x_alone_is_not_written():
         y = torch.empty_like(x)
         mi_adamw.newton_schulz(x, out=y)
     assert torch.equal(y, mi_adamw.newton_schulz(x))
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 60), (150, 200)])
+@pytest.mark.parametrize("ahead", [False, True])
+def test_out_among_the_batch(rows, cols, ahead, monkeypatch):
+    """out begins a matrix, or a row, before or behind x in the same memory."""
+    from mi_adamw import muon
+    monkeypatch.setattr(muon, "_WORKSPACE", 3 * 192 * 256 * 12)    # a few matrices at once
+    for shift in (rows * cols, cols):
+        n = 9
+        store = normal((n + 1) * rows * cols)
+        early, late = (store[s:s + n * rows * cols].view(n, rows, cols) for s in (0, shift))
+        x, out = (early, late) if ahead else (late, early)
+        want = torch.stack([mi_adamw.newton_schulz(m) for m in x.clone()])
+        assert mi_adamw.newton_schulz(x, out=out) is out
+        assert ((out - want).norm() <= 2 * SINGLE * want.norm()).item()
