@@ -1442,7 +1442,7 @@ int mi_adamw_newton_schulz(const void* d_x, int64_t x_batch, int64_t x_row, void
     one.rows = rows;
     one.cols = cols;
     const Cut cut = whole ? Cut{64, 1, 64} : cut_for(&one, 1, batch, single);
-    if (batch * items_of_matrix(rows, cols, MI_ADAMW_NS_TILES, 64, 1) > 0x7fffff)
+    if ((whole ? 1 : items_of_matrix(rows, cols, MI_ADAMW_NS_TILES, 64, 1)) * batch > 0x7fffff)
         return MI_ADAMW_E_INVALID;
     BatchSource src;
     memset(&src, 0, sizeof(src));

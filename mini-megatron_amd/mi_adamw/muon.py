@@ -35,6 +35,7 @@ _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 _PRECISIONS = {"half": _lib.NS_HALF, "single": _lib.NS_SINGLE}
 _SMALL = 128                   # sides up to here run in single precision
 _WORKSPACE = 1 << 30           # bytes of workspace that a batch of matrices may take
+_LAUNCH = (1 << 23) - 1        # matrices that a launch of a workgroup each may take
 _MATRIX_DTYPE = np.dtype([("workspace", "<i8"), ("rows", "<i4"), ("cols", "<i4"),
                           ("lr_ratio", "<f4"), ("reserved", "<i4")])
 assert _MATRIX_DTYPE.itemsize == ctypes.sizeof(_lib.Matrix)
@@ -146,7 +147,7 @@ def newton_schulz(x: torch.Tensor, *, steps: int = 5, coefficients=NS_COEFFICIEN
         with torch.cuda.device(index):
             return newton_schulz(x, steps=steps, coefficients=coefficients, eps=eps,
                                  precision=precision, out=out)
-    at_once = max(1, min(batch, _WORKSPACE // per)) if per else batch
+    at_once = max(1, min(batch, _WORKSPACE // per if per else _LAUNCH))
     ws = torch.empty(at_once * per, dtype=torch.uint8, device=x.device) if per else None
     size = x.element_size()
     stream = torch._C._cuda_getCurrentRawStream(index)

@@ -61,3 +61,16 @@ def test_out_among_the_batch(rows, cols, ahead, monkeypatch):
         want = torch.stack([mi_adamw.newton_schulz(m) for m in x.clone()])
         assert mi_adamw.newton_schulz(x, out=out) is out
         assert ((out - want).norm() <= 2 * SINGLE * want.norm()).item()
+
+
+def test_more_matrices_than_a_launch_takes():
+    for rows, cols in ((1, 1), (2, 3)):
+        x = normal(2 ** 23 + 5, rows, cols)
+        got = mi_adamw.newton_schulz(x)
+        for at in (0, 2 ** 23 - 2, 2 ** 23 - 1, 2 ** 23 + 4):
+            want = mi_adamw.newton_schulz(x[at])
+            assert ((got[at] - want).norm() <= 2 * SINGLE * want.norm()).item()
+        assert torch.isfinite(got).all()
+    # as many, of more 64 x 64 blocks
+    x = normal(2 ** 21, 1, 1).expand(-1, 1, 320)
+    assert torch.isfinite(mi_adamw.newton_schulz(x)).all()
