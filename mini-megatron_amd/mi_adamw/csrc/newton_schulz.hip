@@ -402,10 +402,14 @@ __device__ __forceinline__ const char* uniform(const char* p) {
 // 16 bytes a lane from global memory (a wave-uniform base, a 32-bit offset a lane) to LDS at the
 // wave-uniform byte `to` + lane * 16.  In flight until wait_stages(): the compiler does not count
 // these loads, and would wait for all of them at every read of LDS if it did.
+// (m0 is declared as written, for the compiler's own uses of it; it warns that it reserves m0.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_lds(uint32_t to, const char* base, uint32_t offset) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :: "s"(to), "v"(offset), "s"(base) : "memory");
+                 :: "s"(to), "v"(offset), "s"(base) : "m0", "memory");
 }
+#pragma clang diagnostic pop
 // This wave's loads but the last kLeft have landed and its reads of LDS are done; then the same of
 // the whole workgroup.
 template <int kLeft>
