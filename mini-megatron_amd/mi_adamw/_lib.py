@@ -357,7 +357,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     host.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
                 for name in HOST_BINDINGS))
     host.bind_layer_norm(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
-                           for name in NORM_BINDINGS))
+                           for name in NORM_BINDINGS), MiAdamwError)
     _host = host
     _lib = lib
     return lib

@@ -28,7 +28,7 @@
 //                                       fused=True chain mi_adamw_step*_fused_chain
 //   sync_versions(plan, dict)           dict[id(p)] = (p._version, p.data_ptr())
 //   grads(params, ...)                  what clip_grad_norm_ needs of its gradients
-//   layer_norm(...), bind_layer_norm(addresses)   layer_norm's usual call (norm_host.cpp)
+//   layer_norm(...), bind_layer_norm(addresses, error)   layer_norm's usual call (norm_host.cpp)
 
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>

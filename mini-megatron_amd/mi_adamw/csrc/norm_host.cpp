@@ -12,13 +12,13 @@
 #include <ATen/autocast_mode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
 #include <optional>
-#include <stdexcept>
 #include <string>
 
 #include "mi_adamw.h"
@@ -38,6 +38,7 @@ struct Api {
     const char* (*strerror)(int) = nullptr;
 };
 Api g_api;
+PyObject* g_error = nullptr;        // MiAdamwError
 
 int32_t code_of(at::ScalarType t) {
     return t == at::kBFloat16 ? MI_ADAMW_DTYPE_BF16 : MI_ADAMW_DTYPE_F32;
@@ -48,10 +49,16 @@ void* stream_of(const Tensor& t) {
     return static_cast<void*>(c10::hip::getCurrentHIPStream(t.device().index()).stream());
 }
 
+// MiAdamwError, as mi_adamw._lib.check raises it; a backward calls this without the GIL.
 void check(int code, const char* what) {
-    if (code != MI_ADAMW_OK)
-        throw std::runtime_error(std::string(what) + " failed: " + g_api.strerror(code) +
-                                 " (code " + std::to_string(code) + ")");
+    if (code == MI_ADAMW_OK) return;
+    const std::string text = std::string(what) + " failed: " + g_api.strerror(code) + " (code " +
+                             std::to_string(code) + ")";
+    pybind11::gil_scoped_acquire gil;
+    PyErr_SetString(g_error, text.c_str());
+    python_error error;
+    error.persist();
+    throw error;
 }
 
 struct Results {
@@ -219,7 +226,10 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!g_api.forward || !PyFloat_CheckExact(args[3]) ||
         (args[5] != Py_None && !THPDtype_Check(args[5])))
         Py_RETURN_NONE;
-    try {
+    // every exception keeps its type: a hook's (a checkpoint ends its recomputation by one from
+    // the saving of tensors), the allocator's, the library's
+    HANDLE_TH_ERRORS
+    {
         Tensor x, weight, bias, residual;
         if (!take(args[0], x) || !x.defined() || !take(args[1], weight) || !take(args[2], bias) ||
             !take(args[4], residual))
@@ -262,16 +272,16 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         Py_XDECREF(y);
         Py_XDECREF(s);
         return both;
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-        return nullptr;
     }
+    END_HANDLE_TH_ERRORS
 }
 
-// bind_layer_norm(forward, workspace, grad, strerror): addresses of the library's functions
+// bind_layer_norm(forward, workspace, grad, strerror, error): addresses of the library's functions,
+// and the class of its errors
 PyObject* py_bind_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-    if (nargs != 4) {
-        PyErr_SetString(PyExc_TypeError, "bind_layer_norm(forward, workspace, grad, strerror)");
+    if (nargs != 5 || !PyExceptionClass_Check(args[4])) {
+        PyErr_SetString(PyExc_TypeError,
+                        "bind_layer_norm(forward, workspace, grad, strerror, error)");
         return nullptr;
     }
     void* p[4];
@@ -286,6 +296,8 @@ PyObject* py_bind_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     g_api.workspace = reinterpret_cast<decltype(g_api.workspace)>(p[1]);
     g_api.grad = reinterpret_cast<decltype(g_api.grad)>(p[2]);
     g_api.strerror = reinterpret_cast<decltype(g_api.strerror)>(p[3]);
+    Py_INCREF(args[4]);
+    Py_XSETREF(g_error, args[4]);
     Py_RETURN_NONE;
 }
 

@@ -1,0 +1,105 @@
+"""layer_norm among autograd's other parts: errors keep their types through the native call,
+activation checkpoints, saved-tensor hooks, forward-mode derivatives."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+from torch.utils.checkpoint import checkpoint
+
+import mi_adamw
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def normal(*shape, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.randn(*shape, device=DEV, generator=g)
+
+
+def leaves(rows=24, hidden=96):
+    return [t.requires_grad_(True) for t in (normal(rows, hidden), normal(rows, hidden, seed=1),
+                                             normal(hidden, seed=2), normal(hidden, seed=3))]
+
+
+def norm(x, r, w, b):
+    return mi_adamw.layer_norm(x, w, b, residual=r)
+
+
+def grads(f, ts):
+    y, s = f(*ts)
+    return torch.autograd.grad((y.square().sum() + (s * s.detach().cos()).sum()), ts)
+
+
+@pytest.mark.parametrize("early_stop", [True, False])
+@pytest.mark.parametrize("strided", [False, True])
+def test_activation_checkpoint(early_stop, strided):
+    """The recomputation ends, by an exception from within the norm's own saving of tensors, as soon
+    as everything is there again."""
+    from torch.utils.checkpoint import set_checkpoint_early_stop
+    ts = leaves()
+    if strided:
+        ts[1] = normal(24, 192)[:, ::2].detach().requires_grad_(True)
+    want = grads(norm, ts)
+    with set_checkpoint_early_stop(early_stop):
+        got = grads(lambda *a: checkpoint(norm, *a, use_reentrant=False), ts)
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_an_error_in_a_hook_keeps_its_type():
+    class Mine(Exception):
+        pass
+
+    def refuse(t):
+        raise Mine("no")
+
+    ts = leaves()
+    with pytest.raises(Mine):
+        with torch.autograd.graph.saved_tensors_hooks(refuse, lambda t: t):
+            norm(*ts)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, refuse):
+        y, s = norm(*ts)
+    with pytest.raises(Mine):
+        (y.sum() + s.sum()).backward()
+
+
+@pytest.mark.parametrize("when", ["forward", "backward"])
+def test_out_of_memory_keeps_its_type(when):
+    x = torch.zeros(1 << 18, 1 << 10, device=DEV, requires_grad=True)        # 1 GiB
+    w = torch.ones(1 << 10, device=DEV)
+    if when == "backward":
+        y = mi_adamw.layer_norm(x, w, out_dtype=torch.bfloat16)
+        dy = torch.zeros_like(y)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    room = torch.cuda.memory_reserved() + (256 << 20)
+    torch.cuda.set_per_process_memory_fraction(room / total)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            if when == "forward":
+                mi_adamw.layer_norm(x, w)
+            else:
+                torch.autograd.grad(y, x, dy)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+
+
+@pytest.mark.parametrize("when", ["forward", "backward"])
+def test_a_refusal_of_the_library_is_its_own_error(when):
+    import ctypes
+    from mi_adamw import _lib
+    lib = _lib.load()
+    own = [ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _lib.NORM_BINDINGS]
+    refuse = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p)(
+        lambda args, stream: _lib.E_INVALID)
+    at = ctypes.cast(refuse, ctypes.c_void_p).value
+    ts = leaves()
+    y, s = norm(*ts)
+    try:
+        _lib._host.bind_layer_norm(at, own[1], at, own[3], _lib.MiAdamwError)
+        with pytest.raises(mi_adamw.MiAdamwError, match="invalid argument"):
+            norm(*ts) if when == "forward" else (y.sum() + s.sum()).backward()
+    finally:
+        _lib._host.bind_layer_norm(*own, _lib.MiAdamwError)
+    norm(*ts)[0].sum().backward()
