@@ -42,7 +42,7 @@ def _call(fn, args, device: torch.device, what: str) -> None:
 
 
 def _forward(x, residual, weight, bias, eps, out_dtype, stats: bool):
-    """(y, sum or None, what was normalised as rows, mean, rstd)"""
+    """(y, sum or None, x as rows, mean, rstd)"""
     hidden = x.shape[-1]
     x2 = _as_rows(x, hidden)
     rows = x2.shape[0]
@@ -61,7 +61,7 @@ def _forward(x, residual, weight, bias, eps, out_dtype, stats: bool):
             0 if r2 is None else r2.stride(0), eps, _DTYPES[x.dtype],
             0 if r2 is None else _DTYPES[r2.dtype], _DTYPES[out_dtype])
         _call(_lib.load().mi_adamw_layer_norm, args, x.device, "mi_adamw_layer_norm")
-    return y, total, x2 if total is None else total.view(-1, hidden), mean, rstd
+    return y, total, x2, mean, rstd
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -69,7 +69,8 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, residual, weight, bias, eps, out_dtype):
         y, total, rows, mean, rstd = _forward(x, residual, weight, bias, eps, out_dtype, True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(rows, weight, mean, rstd)
+        # the sum as the output that it is: a view of it would keep it, and with it this node
+        ctx.save_for_backward(rows if total is None else total, weight, mean, rstd)
         ctx.shape, ctx.x_dtype = x.shape, x.dtype
         ctx.residual_dtype = None if residual is None else residual.dtype
         return y if residual is None else (y, total)
@@ -77,11 +78,13 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dsum=None):
-        rows, weight, mean, rstd = ctx.saved_tensors
+        normalised, weight, mean, rstd = ctx.saved_tensors
         need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
         if dy is None and dsum is None:
             return (None,) * 6
-        n, hidden = rows.shape
+        hidden = normalised.shape[-1]
+        rows = _as_rows(normalised, hidden)
+        n = rows.shape[0]
         device = rows.device
         if dy is None:
             dy = torch.zeros(ctx.shape, dtype=torch.float32, device=device)
