@@ -142,7 +142,10 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
         variable_list result(6);
         Tensor dy = grads[0], ds = grads.size() > 1 ? grads[1] : Tensor();
         if (!dy.defined() && !ds.defined()) return result;
-        const auto saved = ctx->get_saved_variables();
+        // a saved-tensor hook may give them back at other strides
+        auto saved = ctx->get_saved_variables();
+        for (Tensor& t : saved)
+            if (t.defined()) t = t.contiguous();
         const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
         const auto x_type = static_cast<at::ScalarType>(ctx->saved_data["x"].toInt());
         const bool with_residual = ctx->saved_data.count("residual") != 0;

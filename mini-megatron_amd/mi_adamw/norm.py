@@ -83,7 +83,9 @@ class _LayerNorm(torch.autograd.Function):
         if dy is None and dsum is None:
             return (None,) * 6
         hidden = normalised.shape[-1]
+        # a saved-tensor hook may give them back at other strides
         rows = _as_rows(normalised, hidden)
+        weight, mean, rstd = (t if t is None else t.contiguous() for t in (weight, mean, rstd))
         n = rows.shape[0]
         device = rows.device
         if dy is None:

@@ -103,3 +103,24 @@ def test_a_refusal_of_the_library_is_its_own_error(when):
     finally:
         _lib._host.bind_layer_norm(*own, _lib.MiAdamwError)
     norm(*ts)[0].sum().backward()
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_saved_tensors_that_come_back_in_another_layout(strided):
+    """A hook gives back the same values, at strides of its own."""
+    ts = leaves()
+    if strided:
+        ts[0] = normal(24, 192)[:, ::2].detach().requires_grad_(True)
+    want = grads(norm, ts)
+
+    def pack(t):
+        return t.dim(), t.t().contiguous() if t.dim() == 2 else torch.stack([t, t], 1)
+
+    def unpack(packed):
+        dim, t = packed
+        return t.t() if dim == 2 else t[:, 0]
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        y, s = norm(*ts)
+    got = torch.autograd.grad((y.square().sum() + (s * s.detach().cos()).sum()), ts)
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
