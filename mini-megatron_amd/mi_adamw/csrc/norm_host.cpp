@@ -2,8 +2,9 @@
 //
 // A small layer norm takes the GPU a few microseconds; through a Python autograd function the
 // host needs 130 us for its forward and backward, here 30.  layer_norm() below returns None for
-// whatever is not the usual call (another device, a strided or empty tensor, a tensor subclass,
-// an argument to refuse), and mi_adamw.norm takes its Python path, which does or reports it.
+// whatever is not the usual call (another device, a strided or empty tensor, a tensor subclass or
+// one with a forward-mode tangent, an argument to refuse), and mi_adamw.norm takes its Python
+// path, which does or reports it.
 
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -215,7 +216,8 @@ bool take(PyObject* o, Tensor& t) {
     if (o == Py_None) return true;
     if (!THPVariable_CheckExact(o)) return false;
     t = THPVariable_Unpack(o);
-    return t.is_cuda() && t.layout() == c10::kStrided && t.is_contiguous() && t.numel() > 0;
+    return t.is_cuda() && t.layout() == c10::kStrided && t.is_contiguous() && t.numel() > 0 &&
+           !t._fw_grad(0).defined();
 }
 
 }  // namespace

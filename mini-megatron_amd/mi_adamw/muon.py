@@ -27,6 +27,7 @@ import torch
 from torch.optim import Optimizer
 
 from . import _lib
+from .norm import refuse_tangents
 from .optimizer import _ROW_DTYPE, _upload
 
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
@@ -103,7 +104,8 @@ def newton_schulz(x: torch.Tensor, *, steps: int = 5, coefficients=NS_COEFFICIEN
     """Orthogonalise a matrix, or each matrix of a 3-D batch, by Newton-Schulz products.
 
     x:          fp32 or bf16 on a ROCm GPU, 2-D or 3-D; rows or columns dense at any stride
-                (other layouts are copied first).  It is not differentiable.
+                (other layouts are copied first).  The result carries no gradient, and a
+                forward-mode tangent is refused.
     precision:  "half", "single", or None: single for fp32, half for bf16.
     out:        where the result goes (same shape, dtype and device; may be x itself or share
                 memory with it).
@@ -120,6 +122,7 @@ def newton_schulz(x: torch.Tensor, *, steps: int = 5, coefficients=NS_COEFFICIEN
     if out is not None and (out.shape != x.shape or out.dtype != x.dtype
                             or out.device != x.device):
         raise ValueError("newton_schulz: out needs x's shape, dtype and device")
+    refuse_tangents("newton_schulz", x, out)
     given = out is not None
     if not given:
         out = torch.empty_like(x)

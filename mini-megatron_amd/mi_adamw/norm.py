@@ -14,6 +14,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -121,6 +122,12 @@ class _LayerNorm(torch.autograd.Function):
                 None, None)
 
 
+def refuse_tangents(what: str, *tensors) -> None:
+    """The kernels compute no forward-mode derivatives: a tangent would be lost without a word."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def _check(x, weight, bias, eps, residual, out_dtype) -> None:
     if x.dim() == 0:
         raise RuntimeError("layer_norm needs at least one dimension to normalise")
@@ -149,6 +156,7 @@ def _check(x, weight, bias, eps, residual, out_dtype) -> None:
         raise ValueError(f"layer_norm: eps should be finite and >= 0 but is: {eps}")
     if x.shape[-1] > 1 << 24 or (x.numel() and x.numel() // x.shape[-1] >= 1 << 23):
         raise NotImplementedError("layer_norm: at most 2^23 - 1 rows of 2^24 values")
+    refuse_tangents("mi_adamw.layer_norm", x, weight, bias, residual)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None = None,

@@ -124,3 +124,42 @@ def test_saved_tensors_that_come_back_in_another_layout(strided):
         y, s = norm(*ts)
     got = torch.autograd.grad((y.square().sum() + (s * s.detach().cos()).sum()), ts)
     assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.parametrize("which", [0, 1, 2, 3])
+@pytest.mark.parametrize("mode", ["no gradient", "gradient", "no_grad"])
+@pytest.mark.parametrize("strided", [False, True])
+def test_forward_mode_derivatives_are_refused(which, mode, strided):
+    ts = [t.detach() for t in leaves()]
+    if strided:
+        ts[0] = normal(24, 192)[:, ::2]
+    if mode == "gradient":
+        ts = [t.requires_grad_(True) for t in ts]
+    norm(*ts)
+    with fwAD.dual_level(), torch.set_grad_enabled(mode != "no_grad"):
+        norm(*ts)
+        ts[which] = fwAD.make_dual(ts[which], torch.ones_like(ts[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            norm(*ts)
+
+
+def test_newton_schulz_refuses_forward_mode():
+    x = normal(20, 30)
+    with fwAD.dual_level():
+        y = mi_adamw.newton_schulz(x)
+        dual = fwAD.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            mi_adamw.newton_schulz(dual)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            mi_adamw.newton_schulz(x, out=fwAD.make_dual(y, torch.ones_like(y)))
+
+
+def test_function_transforms_are_refused():
+    """torch.func's wrappers have no memory of their own: an error, not a wrong number."""
+    x, w = normal(4, 16), normal(16)
+    for f in (lambda a: torch.func.jvp(lambda t: mi_adamw.layer_norm(t, w), (a,), (a,)),
+              lambda a: torch.func.vmap(lambda t: mi_adamw.layer_norm(t, w))(a),
+              lambda a: torch.func.grad(lambda t: mi_adamw.layer_norm(t, w).sum())(a),
+              lambda a: torch.func.jvp(mi_adamw.newton_schulz, (a,), (a,))):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            f(x)
