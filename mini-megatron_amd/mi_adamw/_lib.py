@@ -56,6 +56,8 @@ LR_FLOAT = 0
 LR_VALUE = 1
 LR_DEVICE = 2
 
+FP32_MAX = 3.4028234663852886e38
+
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 

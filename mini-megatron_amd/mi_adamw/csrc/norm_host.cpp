@@ -243,7 +243,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const auto out = args[5] == Py_None
             ? at::autocast::is_autocast_enabled(at::kCUDA) ? at::kFloat : x.scalar_type()
             : reinterpret_cast<THPDtype*>(args[5])->scalar_type;
-        if (!(eps >= 0.0) || !std::isfinite(eps) || x.dim() < 1 || !type_ok(x.scalar_type()) ||
+        if (!(eps >= 0.0) || !std::isfinite(static_cast<float>(eps)) || x.dim() < 1 || !type_ok(x.scalar_type()) ||
             !type_ok(out) || x.size(-1) > (1 << 24) || x.numel() / x.size(-1) >= (1 << 23) ||
             c10::hip::getCurrentHIPStream().device_index() != x.device().index())
             Py_RETURN_NONE;

@@ -58,8 +58,8 @@ def _checked_options(coefficients: tuple, eps: float, steps: int,
         raise ValueError(f"Number of steps must be a positive integer, got {steps}")
     if steps >= 100:
         raise ValueError("Number of steps must be less than 100 for computational efficiency")
-    if not (eps >= 0 and math.isfinite(eps)):
-        raise ValueError(f"eps should be finite and >= 0 but is: {eps}")
+    if not (0 <= eps <= _lib.FP32_MAX):
+        raise ValueError(f"eps should be >= 0 and finite in fp32 but is: {eps}")
     o = _lib.NsOptions(*(float(c) for c in coefficients), eps, steps, precision)
     if _lib.load().mi_adamw_ns_check(ctypes.byref(o)) != _lib.OK:
         raise ValueError(f"Newton-Schulz coefficients {tuple(coefficients)} let singular values "

@@ -152,8 +152,8 @@ def _check(x, weight, bias, eps, residual, out_dtype) -> None:
         if t.dtype != torch.float32:
             raise NotImplementedError(f"layer_norm: {name} of {t.dtype} is not supported (fp32 "
                                       "master parameters only)")
-    if not (eps >= 0 and math.isfinite(eps)):
-        raise ValueError(f"layer_norm: eps should be finite and >= 0 but is: {eps}")
+    if not (0 <= eps <= _lib.FP32_MAX):
+        raise ValueError(f"layer_norm: eps should be >= 0 and finite in fp32 but is: {eps}")
     if x.shape[-1] > 1 << 24 or (x.numel() and x.numel() // x.shape[-1] >= 1 << 23):
         raise NotImplementedError("layer_norm: at most 2^23 - 1 rows of 2^24 values")
     refuse_tangents("mi_adamw.layer_norm", x, weight, bias, residual)

@@ -163,3 +163,12 @@ def test_function_transforms_are_refused():
               lambda a: torch.func.jvp(mi_adamw.newton_schulz, (a,), (a,))):
         with pytest.raises((RuntimeError, NotImplementedError)):
             f(x)
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_an_eps_past_fp32_is_refused(strided):
+    x, w = normal(4, 64), normal(64)
+    x = x[:, ::2] if strided else x[:, :32].contiguous()
+    with pytest.raises(ValueError, match="eps"):
+        mi_adamw.layer_norm(x, w[:32], None, 1e39)
+    assert torch.isfinite(mi_adamw.layer_norm(x, w[:32], None, 3.4e38)).all()
