@@ -110,6 +110,9 @@ def newton_schulz(x: torch.Tensor, *, steps: int = 5, coefficients=NS_COEFFICIEN
     out:        where the result goes (same shape, dtype and device; may be x itself or share
                 memory with it).
     """
+    if torch.compiler.is_compiling():
+        return _untraced(x, steps=steps, coefficients=coefficients, eps=eps, precision=precision,
+                         out=out)
     if x.dim() not in (2, 3):
         raise ValueError(f"newton_schulz takes a matrix or a batch of them, got {x.dim()} "
                          "dimensions")
@@ -166,6 +169,10 @@ def newton_schulz(x: torch.Tensor, *, steps: int = 5, coefficients=NS_COEFFICIEN
     elif given:
         torch.autograd.graph.increment_version(out)     # as an operator that writes it in place
     return out
+
+
+# torch.compile ends its graph here: it cannot trace the library's calls
+_untraced = torch._disable_dynamo(newton_schulz)
 
 
 class _Batch:
