@@ -3,8 +3,8 @@
 // A small layer norm takes the GPU a few microseconds; through a Python autograd function the
 // host needs 130 us for its forward and backward, here 30.  layer_norm() below returns None for
 // whatever is not the usual call (another device, a strided or empty tensor, a tensor subclass or
-// one with a forward-mode tangent, an argument to refuse), and mi_adamw.norm takes its Python
-// path, which does or reports it.
+// one with a forward-mode tangent, under a trace, an argument to refuse), and mi_adamw.norm takes
+// its Python path, which does or reports it.
 
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <optional>
@@ -228,7 +229,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         PyErr_SetString(PyExc_TypeError, "layer_norm(x, weight, bias, eps, residual, out_dtype)");
         return nullptr;
     }
-    if (!g_api.forward || !PyFloat_CheckExact(args[3]) ||
+    if (!g_api.forward || !PyFloat_CheckExact(args[3]) || torch::jit::tracer::isTracing() ||
         (args[5] != Py_None && !THPDtype_Check(args[5])))
         Py_RETURN_NONE;
     // every exception keeps its type: a hook's (a checkpoint ends its recomputation by one from

@@ -27,7 +27,7 @@ import torch
 from torch.optim import Optimizer
 
 from . import _lib
-from .norm import refuse_tangents
+from .norm import refuse_records
 from .optimizer import _ROW_DTYPE, _upload
 
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
@@ -125,7 +125,7 @@ def newton_schulz(x: torch.Tensor, *, steps: int = 5, coefficients=NS_COEFFICIEN
     if out is not None and (out.shape != x.shape or out.dtype != x.dtype
                             or out.device != x.device):
         raise ValueError("newton_schulz: out needs x's shape, dtype and device")
-    refuse_tangents("newton_schulz", x, out)
+    refuse_records("newton_schulz", x, out)
     given = out is not None
     if not given:
         out = torch.empty_like(x)

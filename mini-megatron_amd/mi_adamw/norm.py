@@ -122,8 +122,11 @@ class _LayerNorm(torch.autograd.Function):
                 None, None)
 
 
-def refuse_tangents(what: str, *tensors) -> None:
-    """The kernels compute no forward-mode derivatives: a tangent would be lost without a word."""
+def refuse_records(what: str, *tensors) -> None:
+    """What is lost without a word otherwise: a forward-mode tangent, which the kernels do not
+    compute, and the launches in a trace, which would record the outputs' allocation alone."""
+    if torch.jit.is_tracing():
+        raise NotImplementedError(f"{what} cannot be recorded by torch.jit.trace")
     if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{what} has no forward-mode derivative")
 
@@ -156,7 +159,7 @@ def _check(x, weight, bias, eps, residual, out_dtype) -> None:
         raise ValueError(f"layer_norm: eps should be >= 0 and finite in fp32 but is: {eps}")
     if x.shape[-1] > 1 << 24 or (x.numel() and x.numel() // x.shape[-1] >= 1 << 23):
         raise NotImplementedError("layer_norm: at most 2^23 - 1 rows of 2^24 values")
-    refuse_tangents("mi_adamw.layer_norm", x, weight, bias, residual)
+    refuse_records("mi_adamw.layer_norm", x, weight, bias, residual)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None = None,

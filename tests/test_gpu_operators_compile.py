@@ -1,5 +1,5 @@
 """newton_schulz, layer_norm and Muon called from torch.compile'd functions: they run as they are,
-between the graphs."""
+between the graphs.  A trace refuses them."""
 import pytest
 import torch
 
@@ -66,3 +66,13 @@ def test_module_and_step():
         return [p.detach() for p in model.parameters()]
 
     assert all(torch.equal(a, b) for a, b in zip(run(compiled), run(lambda m: m)))
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_tracing_is_refused(strided):
+    """A trace would record the outputs' allocation and none of the launches."""
+    x, w = normal(4, 64), normal(32)
+    x = x[:, ::2] if strided else x[:, :32].contiguous()
+    for f in (lambda t: mi_adamw.layer_norm(t, w), mi_adamw.newton_schulz):
+        with pytest.raises(NotImplementedError, match="torch.jit.trace"):
+            torch.jit.trace(f, x, check_trace=False)
