@@ -148,3 +148,74 @@ def test_a_backward_through_stepped_copies_raises():
     opt.zero_grad()
     forward().backward()
     opt.step()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_random_sequences(seed):
+    """Eager steps with moved, missing and in-place gradients, options, loaded states and streams
+    that change, replays of graphs recorded along the way: each equals the step of an optimizer built
+    for it alone."""
+    import random
+    rng = random.Random(seed)
+    half = rng.random() < 0.5
+    options = dict(lr=0.02, ns_precision="half" if half else "single")
+    params = make(seed)
+    groups = [{"params": params[:2]}, {"params": params[2:], "nesterov": False}]
+    opt = mi_adamw.Muon(groups, **options)
+    set_grads(params, 0)
+    streams = [torch.cuda.current_stream(), torch.cuda.Stream()]
+    at, graphs = 0, []
+
+    def check(run, grads, settings):
+        # an optimizer of its own, on copies: new tables
+        twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+        twin = mi_adamw.Muon([{"params": twins[:2]}, {"params": twins[2:], "nesterov": False}],
+                             **options)
+        twin.load_state_dict(copy.deepcopy(opt.state_dict()))
+        for group, setting in zip(twin.param_groups, settings):
+            group.update(setting)
+        run()
+        eager(twin, twins, grads)
+        torch.cuda.synchronize()
+        assert same(params, twins)
+        for p, q in zip(params, twins):
+            a, b = (o.state.get(t, {}).get("momentum_buffer") for o, t in ((opt, p), (twin, q)))
+            assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+
+    def settings_now():
+        return [{k: g[k] for k in ("lr", "ns_steps", "weight_decay", "nesterov", "momentum")}
+                for g in opt.param_groups]
+
+    for k in range(25):
+        event = rng.choice(["same", "same", "move", "move", "missing", "options", "load", "stream",
+                            "capture", "replay", "replay"])
+        if event == "stream":
+            at ^= 1
+            streams[at].wait_stream(streams[at ^ 1])
+        with torch.cuda.stream(streams[at]):
+            if event == "move" or any(p.grad is None for p in params):
+                set_grads(params, rng.randrange(1000))
+            if event == "missing":
+                params[rng.randrange(len(params))].grad = None
+            if event == "options":
+                group = rng.choice(opt.param_groups)
+                group["ns_steps"] = rng.choice([3, 5])
+                group["lr"] = rng.choice([0.01, 0.02])
+                group["weight_decay"] = rng.choice([0.0, 0.1])
+            if event == "load":
+                opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+            if event == "replay" and graphs:
+                # a graph steps the momentum it was recorded with
+                graph, grads, settings, moments = rng.choice(graphs)
+                if all(opt.state[p]["momentum_buffer"] is m for p, m in zip(params, moments)):
+                    junk = occupy()
+                    check(graph.replay, grads, settings)
+                    del junk
+                continue
+            check(opt.step, [p.grad for p in params], settings_now())
+            if event == "capture" and all(p.grad is not None for p in params):
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    opt.step()
+                graphs.append((graph, [p.grad for p in params], settings_now(),
+                               [opt.state[p]["momentum_buffer"] for p in params]))
