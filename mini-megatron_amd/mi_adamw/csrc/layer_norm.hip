@@ -260,7 +260,9 @@ __device__ __forceinline__ int32_t sum_dtype(const Fwd& f) {
     return f.x_dtype == kBf16 && f.residual_dtype == kBf16 ? kBf16 : kF32;
 }
 
-// Rows of any length, read again for each sum.
+// Rows of any length, read again for each sum, from the caches while a row fits them: 2048 x 32769
+// bf16 87 us (3.1 TB/s of what has to move), fp32 159 (3.4); 64 x 1048576 bf16 409 (0.66), a quarter
+// of the CUs at work.  Widths past 32768 are no model's here; that there is an answer is the point.
 __global__ __launch_bounds__(kLongThreads) void mi_adamw_layer_norm_long_kernel(Fwd f) {
     __shared__ float lds[2][16];
     const int64_t row = blockIdx.x;
@@ -429,7 +431,9 @@ __global__ __launch_bounds__(kLanes > 256 ? kLanes : 256) void mi_adamw_layer_no
     }
 }
 
-// dx of rows of any length, read twice.
+// dx of rows of any length, read twice: 2048 x 32769 bf16 215 us, fp32 221, with the weights'
+// gradient 361 and 341 (four bytes at a time a lane, two for bf16: 1.1 and 2.4 TB/s of what has to
+// move).
 __global__ __launch_bounds__(kLongThreads) void mi_adamw_layer_norm_long_grad_kernel(Bwd f) {
     __shared__ float lds[32];
     const int64_t row = blockIdx.x, h = f.hidden;
@@ -467,7 +471,7 @@ __global__ __launch_bounds__(kLongThreads) void mi_adamw_layer_norm_long_grad_ke
     }
 }
 
-// Shares of dw and db of long rows: a strip of columns and every gridDim.y-th row.
+// Shares of dw and db of long rows: a strip of columns and every gridDim.y-th row, an element a lane.
 __global__ __launch_bounds__(kStrip) void mi_adamw_layer_norm_long_weight_kernel(Bwd f) {
     const int64_t c = int64_t(blockIdx.x) * kStrip + threadIdx.x, h = f.hidden;
     if (c >= h) return;

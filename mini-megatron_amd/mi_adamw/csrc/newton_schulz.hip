@@ -425,11 +425,11 @@ __device__ __forceinline__ void wait_stages() {
 // barrier a stage.
 //
 // What bounds it: the bytes from L2 to LDS, 8 / kT of a byte for each multiply-add and term.  4096 x
-// 16384, X's launch (tiles of 256): 494 us, 1.11 PFLOP/s beside 9.3 TB/s from L2, 24% of them
-// misses; the whole call 4.63 ms, 3.66 with the products left out (11.7 TB/s) and 3.84 with
+// 16384, X's launch (tiles of 256): 494 to 504 us, 1.09 to 1.11 PFLOP/s beside 9.1 TB/s from L2, 24%
+// of them misses; the whole call 4.63 ms, 3.66 with the products left out (11.7 TB/s) and 3.84 with
 // the loads left out.  S at tiles of 192: 330 us, 830 TFLOP/s.  A fp16 library product of 8192
 // reaches 1.27 PFLOP/s on this card.  With a short sum the results count as well: X of 12 x
-// 768 x 3072 reads and writes 8 bytes an entry, 270 MB in 79 us, at 550 TFLOP/s.
+// 768 x 3072 reads and writes 8 bytes an entry, 226 MB beside its operands in 80 us, at 540 TFLOP/s.
 // Measured steps, 12 x 768 x 3072 and 4096 x 16384, us a call: a stage at a time in tiles of 128, X
 // stored both ways 1453, 7350; the ring, one transposed X, tiles of 256 1173, 6214; the old
 // and new iterate in whole lines 776, 5281; tiles of 192 by rounds, 128 with 4 stages and 8

@@ -1,7 +1,8 @@
 // norm_host.cpp -- layer_norm's usual call in C++: checks, allocation, launch and the autograd node.
 //
-// A small layer norm takes the GPU a few microseconds; through a Python autograd function the
-// host needs 130 us for its forward and backward, here 30.  layer_norm() below returns None for
+// A small layer norm takes the GPU a few microseconds.  Host time of a call with a residual and of
+// its backward, 2048 x 768: 24 and 59 us through a Python autograd function, 7 and 35 here (a
+// product with a vector and its backward: 37 together).  layer_norm() below returns None for
 // whatever is not the usual call (another device, a strided or empty tensor, a tensor subclass or
 // one with a forward-mode tangent, under a trace, an argument to refuse), and mi_adamw.norm takes
 // its Python path, which does or reports it.
