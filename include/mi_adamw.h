@@ -497,8 +497,9 @@ int64_t mi_adamw_ns_workspace(int32_t rows, int32_t cols, int32_t precision);
 int32_t mi_adamw_ns_whole(int32_t rows, int32_t cols);
 
 /* Newton-Schulz of `batch` matrices of one size and dtype (MI_ADAMW_DTYPE_*), rows at
- * x_row and out_row elements (>= cols), matrices at x_batch and out_batch.  d_out may be d_x.
- * At most 2^23 - 1 matrices that mi_adamw_ns_whole() numbers, or 64 x 64 blocks of others.
+ * x_row and out_row elements (>= cols), matrices at x_batch and out_batch.  d_out may be d_x, at
+ * the same distances; other batches may not overlap.  At most 2^23 - 1 matrices that
+ * mi_adamw_ns_whole() numbers, or 64 x 64 blocks of others.
  * d_workspace: batch * mi_adamw_ns_workspace() bytes, 16-byte aligned (NULL if that is 0). */
 int mi_adamw_newton_schulz(const void *d_x, int64_t x_batch, int64_t x_row, void *d_out,
                            int64_t out_batch, int64_t out_row, int32_t batch, int32_t rows,
