@@ -108,7 +108,9 @@ class _MastersAsBf16(torch.autograd.Function):
     def forward(ctx, copies, *masters):
         # the copies come in as one list: only the masters are autograd inputs
         ctx.set_materialize_grads(False)
-        return tuple(c.view_as(c) for c in copies)
+        # not views to autograd, which would refuse them once a step has raised the copies'
+        # versions; they share those, so a backward that saved one before the step still fails
+        return tuple(c.detach() for c in copies)
 
     @staticmethod
     def backward(ctx, *grads):

@@ -150,6 +150,38 @@ def test_a_backward_through_stepped_copies_raises():
     opt.step()
 
 
+@pytest.mark.parametrize("optimizer", [mi_adamw.Muon, mi_adamw.FusedAdamW])
+def test_a_context_held_open_over_steps(optimizer):
+    """The copies are rewritten in place: the forward after a step takes the new weights."""
+    def run(held):
+        torch.manual_seed(0)
+        model = torch.nn.Sequential(torch.nn.Linear(64, 96, bias=False),
+                                    torch.nn.Linear(96, 64, bias=False)).to(DEV)
+        opt = optimizer(model.parameters(), lr=0.02, bf16_copy=True)
+        x = torch.randn(8, 64, device=DEV)
+        losses = []
+
+        def step():
+            opt.zero_grad()
+            loss = model(x).float().square().mean()
+            loss.backward()
+            opt.step()
+            losses.append(loss.item())
+
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            if held:
+                with mi_adamw.bf16_weights(opt, model):
+                    for _ in range(3):
+                        step()
+            else:
+                for _ in range(3):
+                    with mi_adamw.bf16_weights(opt, model):
+                        step()
+        return losses
+
+    assert run(True) == run(False)
+
+
 @pytest.mark.parametrize("seed", range(6))
 def test_random_sequences(seed):
     """Eager steps with moved, missing and in-place gradients, options, loaded states and streams
